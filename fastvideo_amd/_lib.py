@@ -166,7 +166,7 @@ def check(rc: int, what: str) -> None:
         raise RuntimeError(f"{what} failed (rc={rc}): {msg.decode() if msg else '?'}")
 
 
-_TRACE = os.environ.get("FVK_TRACE_CALLS") == "1"   # fault hunts (scripts/guard_sweep.sh): name every call, run it to completion
+_TRACE = os.environ.get("FVK_TRACE_CALLS") == "1"   # name every call on stderr and run it to completion
 
 
 def call(name: str, *args) -> None:

@@ -1,5 +1,4 @@
-// Guard-page device allocator for out-of-bounds hunts: plugs into PyTorch through torch.cuda.memory.CUDAPluggableAllocator
-// (scripts/guard_run.py).  Every allocation gets its OWN virtual-address reservation: whole granules of physical memory mapped at the front, one
+// Guard-page device allocator: plugs into PyTorch through torch.cuda.memory.CUDAPluggableAllocator (tests/_guard.py).  Every allocation gets its OWN virtual-address reservation: whole granules of physical memory mapped at the front, one
 // granule of UNMAPPED address space behind them, and the tensor is placed so that it ENDS where the mapping ends (FVK_GUARD_MODE=front: so that it
 // STARTS where the mapping starts, with the previous reservation's unmapped granule in front of it).  A read or write past the end (or in front of
 // the start) of ANY tensor — by 16 bytes or by gigabytes — is then a GPU page fault ("Memory access fault by GPU ... address 0x...") instead of a
@@ -40,6 +39,15 @@ long g_allocs = 0, g_bytes = 0;
     } while (0)
 }  // namespace
 
+// Where a tensor of `size` bytes lies in a reservation of its own: `mapped` bytes of whole granules, one unmapped granule behind them, the tensor at
+// `offset`.  A function of its own so that the placement can be checked on the host (tests/test_guard_layout.py).
+extern "C" void guard_layout(size_t size, size_t gran, size_t align, int front, size_t* mapped, size_t* reserved, size_t* offset) {
+    const size_t need = (size + align - 1) / align * align;
+    *mapped = (need + gran - 1) / gran * gran;
+    *reserved = *mapped + gran;
+    *offset = front ? 0 : *mapped - need;
+}
+
 extern "C" void* guard_malloc(ssize_t size, int device, hipStream_t) {
     if (size <= 0) size = 1;
     hipMemAllocationProp prop{};
@@ -55,9 +63,8 @@ extern "C" void* guard_malloc(ssize_t size, int device, hipStream_t) {
         fprintf(stderr, "[guard_alloc] granule %zu B, tensor alignment %zu B, tensors placed at the %s of their mapping\n", g_gran, g_align,
                 g_front ? "START" : "END");
     }
-    const size_t need = ((size_t)size + g_align - 1) / g_align * g_align;
-    const size_t mapped = (need + g_gran - 1) / g_gran * g_gran;
-    const size_t reserved = mapped + g_gran;  // one unmapped granule behind the mapping
+    size_t mapped, reserved, offset;
+    guard_layout((size_t)size, g_gran, g_align, g_front, &mapped, &reserved, &offset);
     void* base = nullptr;
     GCHECK(hipMemAddressReserve(&base, reserved, 0, nullptr, 0));
     Rec r{base, reserved, mapped, {}};
@@ -67,7 +74,7 @@ extern "C" void* guard_malloc(ssize_t size, int device, hipStream_t) {
     acc.location = prop.location;
     acc.flags = hipMemAccessFlagsProtReadWrite;
     GCHECK(hipMemSetAccess(base, mapped, &acc, 1));
-    void* p = g_front ? base : (void*)((char*)base + (mapped - need));
+    void* p = (char*)base + offset;
     g_live[p] = r;
     ++g_allocs;
     g_bytes += size;

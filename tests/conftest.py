@@ -23,13 +23,12 @@ def golden_dir():
 
 
 def pytest_collection_modifyitems(config, items):
-    """gpu-marked tests are SKIPPED (not failed) on a box without a HIP device; on a GPU box only a test that faults the GPU
-    on purpose is skipped here, and the ops
-    themselves fail loudly if libfvk_amd.so is missing."""
+    """gpu-marked tests are SKIPPED (not failed) on a box without a HIP device; on a GPU box only a test that asks for a GPU fault
+    is skipped here, and the ops themselves fail loudly if libfvk_amd.so is missing."""
     import torch
-    # This one faults the GPU on purpose (its second half reads 16 bytes behind a mapping), and such a fault can take the card down under every
-    # later test of the run; the runs under the guard allocator that must NOT fault stay on.
-    on_purpose = pytest.mark.skip(reason="faults the GPU on purpose (a read behind the end of a mapping): not run on a card that others use")
+    # Its second half asks scripts/guard_selftest.py for a read behind a mapping, a GPU fault on purpose, which that script no longer makes: the test can only
+    # fail.  Its first half and the placement that makes an overrun meet an unmapped page are tests/test_guard_layout.py's.
+    on_purpose = pytest.mark.skip(reason="asks for a GPU fault on purpose, which nothing in the tree makes any more (see test_guard_layout.py)")
     for item in items:
         if item.nodeid.endswith("test_gpu_guard.py::test_the_detector_detects"):
             item.add_marker(on_purpose)
