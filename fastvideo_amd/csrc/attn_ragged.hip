@@ -604,12 +604,17 @@ __global__ __launch_bounds__(256, 1) void attn_ragged_kernel(fvk_ragged_args a, 
             const int last = place + 1 < to ? place + 1 : to, last_sink = place + 1 < sink_to ? place + 1 : sink_to;
             const bool sees = first < last || sink_from < last_sink;  // some key of this workgroup's part of the walk
             const float l = w.o[qb][8][0];
-            float top = 0.f;  // P up to 2^90 times a value above 2^37 passes fp32 where the quotient does not
+            // P up to 2^90 times a value above 2^37 passes fp32 where the quotient does not.  As bit patterns, so that a NaN counts too (two such
+            // products of opposite sign leave one; a maximum of floats drops it): without the sign, Inf and NaN are the patterns from 0x7f800000 on
+            unsigned top = 0;
 #pragma unroll
             for (int d = 0; d < 8; ++d)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) top = fmaxf(top, __builtin_fabsf(w.o[qb][d][x]));
-            redo[qb] = !(l < L_HIGH) || (l < L_LOW && sees) || ragged_max4(top) == INFINITY;
+                for (int x = 0; x < 4; ++x) {
+                    const unsigned bits = __builtin_bit_cast(unsigned, (float)w.o[qb][d][x]) & 0x7fffffffu;
+                    top = bits > top ? bits : top;
+                }
+            redo[qb] = !(l < L_HIGH) || (l < L_LOW && sees) || ragged_max4(top >= 0x7f800000u ? 1.f : 0.f) > 0.f;
         }
     }
     auto store = [&](bool only_redo) {
