@@ -5,7 +5,8 @@
 namespace {
 
 // ------------------------------------------------------------------ plan
-// All whole numbers.  With total = start + new, pages = ceil(total / P), need = max(0, pages - held):
+// All whole numbers.  With new = the request's tokens that the batch holds (those beyond n_tokens are dropped: they have no row, so no key and no page),
+// total = start + new, pages = ceil(total / P), need = max(0, pages - held):
 //   a request is GRANTED iff its pages fit the table's width and (need = 0 or (sum of the needs before it) + need <= free_count);
 //   its i-th new page is free[count - 1 - off - i];  a page is dead once no row of this step or a later one can see it (window, sink) and goes back
 //   onto the stack in (request, page) order.
@@ -28,11 +29,12 @@ struct PlanReq {
     int start, add, pages, need, held, fits;
 };
 
-__device__ __forceinline__ PlanReq plan_req(const PlanArgs& a, int r) {
+// add: rows of the batch that the request has, cu[r + 1] - cu[r]
+__device__ __forceinline__ PlanReq plan_req(const PlanArgs& a, int r, int add) {
     PlanReq q;
-    const int s = a.starts[r], n = a.new_lens[r], h = a.held[r];
+    const int s = a.starts[r], h = a.held[r];
     q.start = s > 0 ? s : 0;
-    q.add = n > 0 ? (n < a.n_tokens ? n : a.n_tokens) : 0;
+    q.add = add;
     q.held = h > 0 ? h : 0;
     q.total = (long)q.start + q.add;
     const long pages = (q.total + a.page - 1) / a.page;
@@ -61,8 +63,8 @@ __device__ __forceinline__ int plan_page(const PlanArgs& a, const PlanReq& q, in
     return a.table[(long)r * a.width + j];
 }
 
-// Exclusive prefix sums over the requests of (new tokens, needed pages), by the whole workgroup (256 threads), into cu[0..R] (clamped to n_tokens)
-// and off[0..R].
+// Exclusive prefix sums over the requests by the whole workgroup (256 threads): new tokens, clamped to n_tokens, into cu[0..R], and the pages that the
+// tokens within the batch need into off[0..R].
 __device__ void plan_scan(const PlanArgs& a, int* cu, int* off) {
     __shared__ long wsum_t[4];
     __shared__ int wsum_p[4];
@@ -72,32 +74,40 @@ __device__ void plan_scan(const PlanArgs& a, int* cu, int* off) {
     for (int r0 = 0; r0 < a.R; r0 += 256) {
         const int r = r0 + tid;
         long t = 0;
-        int p = 0;
         if (r < a.R) {
-            const PlanReq q = plan_req(a, r);
-            t = q.add;
-            p = q.need;
+            const int n = a.new_lens[r];
+            t = n > 0 ? n : 0;
         }
         const long t0 = t;
-        const int p0 = p;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const long tu = __shfl_up(t, o, 64);
-            const int pu = __shfl_up(p, o, 64);
-            if (lane >= o) { t += tu; p += pu; }
+            if (lane >= o) t += tu;
         }
-        if (lane == 63) { wsum_t[wave] = t; wsum_p[wave] = p; }
+        if (lane == 63) wsum_t[wave] = t;
         __syncthreads();
         long bt = base_t;
+        for (int w = 0; w < 4; ++w) {
+            if (w < wave) bt += wsum_t[w];
+            base_t += wsum_t[w];
+        }
+        const long from = bt + t - t0 < a.n_tokens ? bt + t - t0 : a.n_tokens, to = bt + t < a.n_tokens ? bt + t : a.n_tokens;
+        int p = r < a.R ? plan_req(a, r, (int)(to - from)).need : 0;
+        const int p0 = p;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int pu = __shfl_up(p, o, 64);
+            if (lane >= o) p += pu;
+        }
+        if (lane == 63) wsum_p[wave] = p;
+        __syncthreads();
         int bp = base_p;
         for (int w = 0; w < 4; ++w) {
-            if (w < wave) { bt += wsum_t[w]; bp += wsum_p[w]; }
-            base_t += wsum_t[w];
+            if (w < wave) bp += wsum_p[w];
             base_p += wsum_p[w];
         }
         if (r < a.R) {
-            const long c = bt + t - t0;
-            cu[r] = (int)(c < a.n_tokens ? c : a.n_tokens);
+            cu[r] = (int)from;
             off[r] = bp + p - p0;
         }
         __syncthreads();
@@ -117,10 +127,10 @@ __device__ __forceinline__ int plan_count(const PlanArgs& a) {
 }
 
 // pages taken off the stack: the granted needs form a prefix of the requests (the first refusal of a need refuses every later one)
-__device__ int plan_taken(const PlanArgs& a, const int* off, int count) {
+__device__ int plan_taken(const PlanArgs& a, const int* cu, const int* off, int count) {
     int lo = 0;
     for (int r = threadIdx.x; r < a.R; r += 256) {
-        const PlanReq q = plan_req(a, r);
+        const PlanReq q = plan_req(a, r, cu[r + 1] - cu[r]);
         if (q.need > 0 && plan_granted(q, off[r], count) && off[r] + q.need > lo) lo = off[r] + q.need;
     }
     __shared__ int best[4];
@@ -146,7 +156,7 @@ __global__ __launch_bounds__(256) void paged_plan_kernel(PlanArgs a) {
         const bool shared = a.row_waves > 1;
         const int r = shared ? blockIdx.x : blockIdx.x * 4 + (tid >> 6), lane = shared ? tid : tid & 63, step = shared ? 256 : 64;
         if (r >= a.R) return;  // (a shared row's workgroup has one request: all of it leaves)
-        const PlanReq q = plan_req(a, r);
+        const PlanReq q = plan_req(a, r, cu[r + 1] - cu[r]);
         const bool ok = plan_granted(q, off[r], count);
         int first, last, dead = 0;
         plan_dead_range(a, q, first, last);
@@ -182,7 +192,7 @@ __global__ __launch_bounds__(256) void paged_plan_kernel(PlanArgs a) {
     }
     const int block = blockIdx.x - a.table_blocks, blocks = gridDim.x - a.table_blocks;
     if (block == 0) {
-        const int taken = plan_taken(a, off, count);
+        const int taken = plan_taken(a, cu, off, count);
         if (tid == 0) {
             a.count_out[0] = count - taken;  // the second launch adds the dead pages
             if (a.scratch) a.scratch[2 * a.R] = count - taken;
@@ -199,7 +209,7 @@ __global__ __launch_bounds__(256) void paged_plan_kernel(PlanArgs a) {
                 if (cu[mid] <= i) lo = mid;
                 else hi = mid;
             }
-            const PlanReq q = plan_req(a, lo);
+            const PlanReq q = plan_req(a, lo, cu[lo + 1] - cu[lo]);
             const long at = (long)q.start + (i - cu[lo]);
             pos = (int)(at < 0x7fffffffL ? at : 0x7fffffffL);
             if (plan_granted(q, off[lo], count)) {
@@ -237,7 +247,7 @@ __global__ __launch_bounds__(256) void paged_release_kernel(PlanArgs a) {
         all += __shfl_xor(all, o, 64);
     }
     if (r == 0 && lane == 0) a.count_out[0] = left + all < a.n_free ? left + all : a.n_free;
-    const PlanReq q = plan_req(a, r);
+    const PlanReq q = plan_req(a, r, a.cu_q[r + 1] - a.cu_q[r]);  // (of the first launch)
     int first, last, at = left + before;
     plan_dead_range(a, q, first, last);
     if (a.scratch[r] == 0) return;  // nothing dead, or not granted

@@ -934,7 +934,8 @@ def paged_plan(starts, new_lens, block_table, pages_held, free_pages, free_count
                causal=False) -> PagedPlan:
     """Block tables, slot map, key lengths and (t, h, w) positions of a step, from the requests' lengths, on the GPU (fvk_paged_plan).
     starts / new_lens / pages_held int32 [R], block_table int32 [R, W], free_pages int32 [F] (a stack: entries [0, free_count) are free, F = the pool's
-    pages), free_count int32 [1].  n_tokens: rows of the step's packed batch (>= the sum of new_lens; the rest are padding rows with slot -1).
+    pages), free_count int32 [1].  n_tokens: rows of the step's packed batch (>= the sum of new_lens: the rest are padding rows with slot
+    -1; below it: tokens without a row are not planned, neither their pages nor their place in kv_lens).
     Nothing is read back: a request whose pages do not fit has granted = 0, kv_len = 0 and slots -1, and its table row stays as it was.
     window / sink / causal as in attn_paged: pages that no row can see any more go back onto the stack.  Returns new tensors (the inputs stay)."""
     fast = _fast(block_table)

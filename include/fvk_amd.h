@@ -418,7 +418,8 @@ int fvk_mfma_sustained_probe_bf16(float* out, int workgroups, int iters, int dat
  * (ref: fastvideo/models/dits/causal_wanvideo.py:123-173); here a window with sink tokens leaves the old pages and the shift is gone. */
 
 /* The plan of a step, from the requests' lengths, on the GPU (whole numbers; nothing is read back).  Per request r: starts[r] tokens are cached,
- * new_lens[r] are added (re-writing the same tokens = the same starts again), total = start + new, pages = ceil(total / page_size),
+ * new_lens[r] are added (re-writing the same tokens = the same starts again); new = those of them that the batch's n_tokens rows hold, in request order
+ * (the rest have no row: no key, no page, no length), total = start + new, pages = ceil(total / page_size),
  * need = max(0, pages - pages_held[r]).
  *   granted[r]   = pages <= table_width and (need = 0 or the needs of requests 0..r together <= free_count)
  *   table_out    : block_table with granted request r's i-th new page = free_pages[free_count - 1 - (needs before r) - i]; dead pages become -1
@@ -430,7 +431,7 @@ int fvk_mfma_sustained_probe_bf16(float* out, int workgroups, int iters, int dat
  *   positions [n_tokens, 3]: (time, height, width) of the token's place on a grid of grid_h x grid_w tokens per frame (1 x 1: a plain counter)
  * A page of a granted request is dead when no row of this step or a later one sees it: window > 0, page begin >= sink, page end <= total - window
  * (causal: total - new + 1 - window).  dead_counts [2 * n_requests + 1]: scratch, needed when window > 0.  Outputs must not alias inputs.
- * n_requests <= 4096.  Negative lengths count as 0; tokens beyond n_tokens are dropped. */
+ * n_requests <= 4096.  Negative lengths count as 0. */
 int fvk_paged_plan(const int32_t* starts, const int32_t* new_lens, const int32_t* block_table, const int32_t* pages_held,
                    const int32_t* free_pages, const int32_t* free_count, int32_t* table_out, int32_t* held_out, int32_t* free_out,
                    int32_t* count_out, int32_t* cu_q, int32_t* kv_lens, int32_t* slot_map, int32_t* positions, int32_t* granted,
