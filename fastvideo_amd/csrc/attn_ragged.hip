@@ -470,9 +470,9 @@ __global__ __launch_bounds__(256, 1) void attn_ragged_kernel(fvk_ragged_args a, 
         q_ok[qb] = row <= last_row;
         qrow[qb] = q_ok[qb] ? row : last_row;
         const bf16_t* qp = (const bf16_t*)a.q + (long)(rq.q0 + qrow[qb]) * a.q_ts + (long)h * a.q_hs;
-        // straight into the accumulator file; the prologue's vmcnt(0) covers them
+        // in front of the first LDS-DMA piece, so that they arrive behind the set-up
 #pragma unroll
-        for (int c = 0; c < 4; ++c) asm volatile("global_load_dwordx4 %0, %1, off" : "=a"(w.qf[qb][c]) : "v"(qp + c * 32 + g * 8) : "memory");
+        for (int c = 0; c < 4; ++c) w.qf[qb][c] = ld_bf16x8(qp + c * 32 + g * 8);
     }
     Edges e;
     e.causal = a.causal;
@@ -540,6 +540,10 @@ __global__ __launch_bounds__(256, 1) void attn_ragged_kernel(fvk_ragged_args a, 
         ta = 2 * (ks.n_sink - st0) + (from > ks.lo16 ? (from - ks.lo16 + 63) / 64 : 0);
         tb = 2 * (ks.n_sink - st0) + (to > ks.lo16 ? (to - ks.lo16) / 64 : 0);
     }
+    // Q into the accumulator file: a use that the compiler waits for (an asm load's register counts as written at once, and may be copied or spilled before
+    // it is); the fence behind it pads these writes against the first MFMA
+#pragma unroll
+    for (int qb = 0; qb < 4; ++qb) asm volatile("" : "+a"(w.qf[qb][0]), "+a"(w.qf[qb][1]), "+a"(w.qf[qb][2]), "+a"(w.qf[qb][3]));
     w.fence_o();
     WAIT_ALL()
     BAR()
