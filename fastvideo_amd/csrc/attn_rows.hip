@@ -31,9 +31,9 @@ constexpr int rows_lds(int qb, int stages) {
     return ring > merge ? ring : merge;
 }
 
-template <int QB, bool PAGED>
-__global__ __launch_bounds__(256, QB <= 2 ? 2 : 1) void attn_rows_kernel(fvk_ragged_args a, RaggedParts part, int flat, int stages) {
 #if defined(__HIP_DEVICE_COMPILE__)
+template <int QB, bool PAGED, int STAGES>
+__device__ __forceinline__ void attn_rows(const fvk_ragged_args& a, const RaggedParts& part, int flat) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256, QB <= 2 ? 2 : 1) void attn_rows_kernel(fvk_rag
     const float c2 = a.scale * 1.4426950408889634f;
     const bf16_t* kb = (const bf16_t*)a.k + (long)kvh * a.k_hs + (PAGED ? 0L : (long)rq.k0 * a.k_rs);
     const bf16_t* vb = (const bf16_t*)a.v + (long)kvh * a.v_hs + (PAGED ? 0L : (long)rq.k0 * a.v_rs);
-    unsigned char* ring = smem + wave * stages * STAGE_BYTES;
+    unsigned char* ring = smem + wave * STAGES * STAGE_BYTES;
     RaggedPages pages;
     if (PAGED) pages.init(a, r);
     // LDS-DMA: instruction i of 16 rows writes rows 4i .. 4i+3 (lane >> 4) linearly, so a lane fetches the chunk that belongs at its place
@@ -136,9 +136,9 @@ __global__ __launch_bounds__(256, QB <= 2 ? 2 : 1) void attn_rows_kernel(fvk_rag
 
         int s = st0 + wave;
         if (s < st1) issue(s, 0);
-        if (stages > 1 && s + 4 < st1) issue(s + 4, 1);
-        for (int slot = 0; s < st1; s += 4, slot ^= stages - 1) {
-            if (stages > 1 && s + 4 < st1) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");  // the 16 pieces of the next stage may still fly
+        if (STAGES > 1 && s + 4 < st1) issue(s + 4, 1);
+        for (int slot = 0; s < st1; s += 4, slot ^= STAGES - 1) {
+            if (STAGES > 1 && s + 4 < st1) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");  // the 16 pieces of the next stage may still fly
             else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __builtin_amdgcn_sched_barrier(0);
             const unsigned char* kl = ring + slot * STAGE_BYTES;
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(256, QB <= 2 ? 2 : 1) void attn_rows_kernel(fvk_rag
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read
             __builtin_amdgcn_sched_barrier(0);
-            if (s + 4 * stages < st1) issue(s + 4 * stages, slot);
+            if (s + 4 * STAGES < st1) issue(s + 4 * STAGES, slot);
         }
 
         // ---- merge the four waves: each leaves (O, m, l) of its rows
@@ -264,6 +264,27 @@ __global__ __launch_bounds__(256, QB <= 2 ? 2 : 1) void attn_rows_kernel(fvk_rag
         if (flat) break;
         __syncthreads();
     }
+}
+#endif
+
+// The two-stage ring: MFMAs while the wave's own LDS-DMA pieces fly, one workgroup per compute unit (128 KB of LDS), so one wave per SIMD: it owns the
+// register file (fvk_common.h: FVK_CLAIM_WHOLE_REGISTER_FILE), whatever its 123 .. 471 registers would leave to a neighbour.
+template <int QB, bool PAGED>
+__global__ __launch_bounds__(256, 1) void attn_rows_ring_kernel(fvk_ragged_args a, RaggedParts part, int flat) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    FVK_CLAIM_WHOLE_REGISTER_FILE();
+    attn_rows<QB, PAGED, 2>(a, part, flat);
+#endif
+}
+
+// One stage: a wave has waited for all its pieces before its first MFMA.  Two workgroups of the smaller tiles share a compute unit and claim half of the
+// register file each; the 64-row tile is alone and claims all of it.
+template <int QB, bool PAGED>
+__global__ __launch_bounds__(256, QB <= 2 ? 2 : 1) void attn_rows_kernel(fvk_ragged_args a, RaggedParts part, int flat) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    if (QB <= 2) asm volatile("" ::: "v255");
+    else FVK_CLAIM_WHOLE_REGISTER_FILE();
+    attn_rows<QB, PAGED, 1>(a, part, flat);
 #endif
 }
 
@@ -334,16 +355,20 @@ __global__ __launch_bounds__(256) void ragged_merge_kernel(fvk_ragged_args a, Ra
 
 template <int QB, bool PAGED>
 int launch_rows(const fvk_ragged_args* a, const RaggedParts& part, long row_blocks, hipStream_t s) {
-    static FvkLdsConfigured configured;
-    if (int rc = fvk_config_lds(configured, (const void*)attn_rows_kernel<QB, PAGED>, rows_lds(QB, 2), "fvk_attn_ragged_bf16 (rows)")) return rc;
+    static FvkLdsConfigured one, ring;
     // parts of at most four stages by the host's bound: a ring of one stage, so that two workgroups fit a compute unit
     const int stages = (long)a->max_kv <= 4L * ST * part.n ? 1 : 2;
+    if (int rc = stages == 1 ? fvk_config_lds(one, (const void*)attn_rows_kernel<QB, PAGED>, rows_lds(QB, 1), "fvk_attn_ragged_bf16 (rows)")
+                             : fvk_config_lds(ring, (const void*)attn_rows_ring_kernel<QB, PAGED>, rows_lds(QB, 2), "fvk_attn_ragged_bf16 (rows)"))
+        return rc;
     // several tiles in some request: one workgroup per tile of the batch (at most T * G / tile + R of them), as long as gridDim.z holds them
     const long tiles = (long)a->T * (a->H / a->Hkv) / (16 * QB) + a->R;
     const bool flat = a->R > 1 && row_blocks > 1 && tiles <= 65535;
     const long cap = 65535 / a->Hkv;  // gridDim.y; the kernel walks on where there are more
     const unsigned y = flat ? a->Hkv : (unsigned)(a->Hkv * (row_blocks < cap ? row_blocks : cap));
-    hipLaunchKernelGGL((attn_rows_kernel<QB, PAGED>), dim3(part.n, y, flat ? (unsigned)tiles : (unsigned)a->R), dim3(256), rows_lds(QB, stages), s, *a, part, (int)flat, stages);
+    const dim3 grid(part.n, y, flat ? (unsigned)tiles : (unsigned)a->R);
+    if (stages == 1) hipLaunchKernelGGL((attn_rows_kernel<QB, PAGED>), grid, dim3(256), rows_lds(QB, 1), s, *a, part, (int)flat);
+    else hipLaunchKernelGGL((attn_rows_ring_kernel<QB, PAGED>), grid, dim3(256), rows_lds(QB, 2), s, *a, part, (int)flat);
     FVK_LAUNCH_CHECK();
     return FVK_OK;
 }

@@ -36,3 +36,30 @@ def test_the_rule_knows_such_a_load():
     assert not loads_into_registers('"global_load_dwordx4 %0, %1, off\\n\\ts_waitcnt vmcnt(0)" : "=a"(x) : "v"(p) : "memory"')
     assert not loads_into_registers('"buffer_load_dwordx4 %4, s[96:99], 0 offen lds" : : "v"(at) : "memory"')
     assert not loads_into_registers('"s_waitcnt vmcnt(0)" ::: "memory"')
+
+
+def kernels(tmp_path, names):
+    """name -> (registers of a wave, spilled vector registers) of the built library's kernels."""
+    import subprocess
+    import test_register_claims as claims
+    objcopy, readelf = os.path.join(claims.LLVM, "llvm-objcopy"), os.path.join(claims.LLVM, "llvm-readelf")
+    if not (os.path.exists(claims.LIB) and os.path.exists(objcopy) and os.path.exists(readelf)):
+        pytest.skip("library not built or no llvm tools")
+    fat, seen = str(tmp_path / "fat.bin"), {}
+    subprocess.run([objcopy, "--dump-section", f".hip_fatbin={fat}", claims.LIB, str(tmp_path / "copy.so")], check=True)
+    for i, elf in enumerate(claims._device_elfs(open(fat, "rb").read())):
+        f = tmp_path / f"co{i}.elf"
+        f.write_bytes(elf)
+        for blk in subprocess.run([readelf, "--notes", str(f)], capture_output=True, text=True).stdout.split("- .agpr_count:")[1:]:
+            name = re.search(r"\.name:\s+(\S+)", blk).group(1)
+            if any(n in name for n in names):
+                seen[name] = tuple(int(re.search(rf"\.{k}:\s+(\d+)", blk).group(1)) for k in ("vgpr_count", "vgpr_spill_count"))
+    return seen
+
+
+def test_rows_kernels_leave_no_room_beside_them(tmp_path):
+    """One workgroup per compute unit (the two-stage ring, the 64-row tile): all 512 registers of a SIMD.  Two of them: half each."""
+    ring = kernels(tmp_path, ["attn_rows_ring_kernel"])
+    assert len(ring) == 6 and all(v == (512, 0) for v in ring.values()), ring
+    one = kernels(tmp_path, ["attn_rows_kernel"])
+    assert len(one) == 6 and all(v == ((512 if "ILi4E" in n else 256), 0) for n, v in one.items()), one
