@@ -1,5 +1,5 @@
 // What the kernels of the ragged attention family share (attn_rows.hip: few rows per request; attn_ragged.hip: blocks of rows): the argument
-// block, the key range of a run of rows and the stages that cover it, and the LDS-DMA of 16 key rows from a page (or from packed rows).
+// block, the key range of a run of rows and the stages that cover it (ragged_walk.h), and the LDS-DMA of 16 key rows from a page (or from packed rows).
 //
 // The batch is packed: request r owns q rows [cu_q[r], cu_q[r+1]) and either the first kv_lens[r] tokens of its pages (block_table row r) or
 // the rows [cu_k[r], cu_k[r+1]) of packed k / v.  Row i of nq rows has the place p = len - 1 (all rows see the whole cache) or
@@ -9,6 +9,7 @@
 // outside the tensors.  A page id outside the pool reads as zero rows (its buffer descriptor has no records).
 #pragma once
 #include "fvk_common.h"
+#include "ragged_walk.h"
 
 namespace fvk {
 
@@ -35,60 +36,6 @@ __device__ __forceinline__ int wave_scan(int v) {
     return v;
 }
 __device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
-__device__ __forceinline__ int clamp_i(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
-
-struct RaggedReq {
-    int q0, nq;  // first row, rows
-    int k0, len; // packed keys: first row; keys
-};
-
-template <bool PAGED>
-__device__ __forceinline__ RaggedReq ragged_req(const fvk_ragged_args& a, int r) {
-    RaggedReq q;
-    q.q0 = clamp_i(a.cu_q[r], 0, a.T);
-    const int q1 = clamp_i(a.cu_q[r + 1], 0, a.T);
-    q.nq = q1 > q.q0 ? q1 - q.q0 : 0;
-    if (PAGED) {
-        q.k0 = 0;
-        q.len = clamp_i(a.kv_lens[r], 0, a.table_width << a.page_shift);
-    } else {
-        q.k0 = clamp_i(a.kv_lens[r], 0, a.total_k);
-        const int k1 = clamp_i(a.kv_lens[r + 1], 0, a.total_k);
-        q.len = k1 > q.k0 ? k1 - q.k0 : 0;
-    }
-    return q;
-}
-
-// The keys that some row of the token run [i0, i1] sees, as [0, sink_end) and [lo, hi), in stages of STAGE keys; keys in [full_lo, full_hi) of the
-// second part are seen by every row of the run (those of the first part by every row whose place is behind them: full_hi again).
-struct RaggedKeys {
-    int sink_end, lo, hi, lo16, n_sink, n;  // n stages, the first n_sink of them over [0, sink_end)
-    int full_lo, full_hi;
-};
-
-template <int STAGE>
-__device__ __forceinline__ RaggedKeys ragged_keys(const fvk_ragged_args& a, const RaggedReq& q, int i0, int i1) {
-    RaggedKeys k;
-    const int p0 = a.causal ? q.len - q.nq + i0 : q.len - 1, p1 = a.causal ? q.len - q.nq + i1 : q.len - 1;
-    k.hi = p1 + 1 > 0 ? p1 + 1 : 0;
-    k.lo = 0;
-    k.sink_end = 0;
-    k.full_lo = 0;
-    k.full_hi = p0 + 1 > 0 ? p0 + 1 : 0;
-    if (a.window > 0) {
-        const int lo = p0 - a.window + 1, last = p1 - a.window + 1;
-        k.lo = lo > 0 ? lo : 0;
-        k.full_lo = last > 0 ? last : 0;
-        if (a.sink >= k.lo) k.lo = 0;  // one run of keys
-        else k.sink_end = a.sink;
-        if (a.sink >= k.full_lo) k.full_lo = 0;
-    }
-    k.lo16 = k.lo & ~15;
-    k.n_sink = (k.sink_end + STAGE - 1) / STAGE;
-    k.n = k.n_sink + (k.hi > k.lo16 ? (k.hi - k.lo16 + STAGE - 1) / STAGE : 0);
-    return k;
-}
-
 // 1 KB from memory to LDS: 16 bytes per lane from base + 16 * off16 + at (zeros where that passes `records` bytes behind base + 16 * off16), to lds + 16 * lane.
 // Written out because a ds_read_b64_tr_b16 behind the builtin makes the compiler wait for ALL loads in flight (vmcnt(0) in front of every V fragment; the
 // block kernel ran at half its rate with it): it cannot know that the fragment's ring slot is another one.  The waits are the kernels' own: counted vmcnt.
@@ -118,10 +65,6 @@ __device__ __forceinline__ float ragged_max4(float v) {
     const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
     return fmaxf(__builtin_bit_cast(float, (unsigned)b[0]), __builtin_bit_cast(float, (unsigned)b[1]));
 }
-
-// first key of stage s
-template <int STAGE>
-__device__ __forceinline__ int ragged_stage(const RaggedKeys& k, int s) { return s < k.n_sink ? s * STAGE : k.lo16 + (s - k.n_sink) * STAGE; }
 
 // Page ids of one request, 64 at a time in a register (lane i: page first + i): an id is one v_readlane away, and the table is read once per 64 pages.
 struct RaggedPages {

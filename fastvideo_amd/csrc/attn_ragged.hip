@@ -34,7 +34,7 @@ using namespace fvk;
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int BMQ = 256;
+constexpr int BMQ = RAGGED_BLOCK;
 constexpr int KT = 128;              // keys per stage
 constexpr int TILE = KT * 256;       // one stage of K or V
 constexpr int V_BASE = 2 * TILE;
@@ -312,30 +312,20 @@ struct Wave {
 
 // The groups of eight stages from `first` on, one per lane: page-table entry (a load), then offset and records.
 template <bool PAGED>
-struct Groups {
+struct Groups : RaggedGroups {
     const int32_t* row;
-    int width, shift, n_pages, end;  // end: one past the last stage of this workgroup
-    unsigned ps16, rs16, rs2;        // page and row stride in 16-byte units, row stride in bytes
-    unsigned base16;                 // packed keys: the request's first row
 
-    __device__ __forceinline__ int key_of(const RaggedKeys& ks, int first) const {
-        const int lane = threadIdx.x & 63;
-        return ragged_stage<KT>(ks, first + (lane >> 3)) + 16 * (lane & 7);
-    }
     __device__ __forceinline__ int load(const RaggedKeys& ks, int first) const {
         if (!PAGED) return 0;
-        const int index = key_of(ks, first) >> shift;
-        const bool in = first + (int)((threadIdx.x & 63) >> 3) < end && index < width;
-        return in ? row[in ? index : 0] : -1;
+        const int lane = threadIdx.x & 63, st = first + (lane >> 3), k = key<KT>(ks, st, lane & 7);
+        const bool in = in_table(st, k);
+        return in ? row[in ? k >> shift : 0] : -1;
     }
     __device__ __forceinline__ void set(const RaggedKeys& ks, int first, int page, int& off, int& rec) const {
-        const int st = first + (int)((threadIdx.x & 63) >> 3), key = key_of(ks, first);
-        const int left = (st < ks.n_sink ? ks.sink_end : ks.hi) - key;
-        const bool ok = st < end && left > 0 && (!PAGED || (page >= 0 && page < n_pages));
-        const int rows = left < 16 ? left : 16;
-        off = PAGED ? (int)((unsigned)page * ps16 + (unsigned)(key & ((1 << shift) - 1)) * rs16) : (int)(base16 + (unsigned)key * rs16);
-        off = ok ? off : 0;
-        rec = ok ? (int)((rows - 1) * rs2 + 256) : 0;
+        const int lane = threadIdx.x & 63, st = first + (lane >> 3);
+        const RaggedGroup g = at<PAGED>(ks, st, key<KT>(ks, st, lane & 7), page);
+        off = g.off;
+        rec = g.rec;
     }
 };
 
@@ -346,10 +336,6 @@ __global__ __launch_bounds__(256, 1) void attn_ragged_kernel(fvk_ragged_args a, 
     FVK_CLAIM_WHOLE_REGISTER_FILE();
     const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // Workgroup x lands on XCD x % 8 (its own L2).  Heads go in teams of four key heads; within every eight ranks (see below) the pairs (head, place in the
-    // eight) are dealt to the XCDs in runs of H, team by team.  So an XCD works on a few heads, whose blocks read the same pages, but on four key heads
-    // rather than one: rows of one head lie Hkv * 256 bytes apart and touch only some of the L2's channels.  No gaps: a workgroup without work in front
-    // of others leaves a compute unit empty (the dispatcher deals in fixed turns: 228 blocks of equal length took two rounds of 256 with gaps).
     RaggedReq mine = {0, 0, 0, 0};  // up to 64 requests: request `lane`
     int blocks = 0, total;
     const bool few = a.R <= 64;
@@ -360,47 +346,16 @@ __global__ __launch_bounds__(256, 1) void attn_ragged_kernel(fvk_ragged_args a, 
     } else {
         total = total_blocks<PAGED>(a);
     }
-    const int xcd = blockIdx.x & 7, full = total >> 3, G = a.H / a.Hkv, G4 = 4 * G;
-    // tasks of an XCD: for every run of the key axis the pairs of the whole eights, then its share of all runs' pairs of the last, incomplete eight
-    const int rem = total & 7, whole = full * a.H, left_over = a.H * rem, local = blockIdx.x >> 3;
-    int run, row = full, wide = rem, pair, h, rank;
-    if (local < whole * part.n) {
-        run = part.n > 1 ? local / whole : 0;
-        pair = local - run * whole;
-        row = pair / a.H;
-        wide = 8;
-        pair += ((row & 1 ? 7 - xcd : xcd) - row) * a.H;  // back and forth: ranks descend in cost
-    } else {
-        pair = (int)((long)xcd * left_over * part.n >> 3) + local - whole * part.n;
-        if (pair >= (int)((long)(xcd + 1) * left_over * part.n >> 3)) return;  // the host's bound on the number of blocks is not tight
-        run = part.n > 1 ? pair / left_over : 0;
-        pair -= run * left_over;
-    }
-    {
-        // pair number, team-major: (team, place, member)
-        const int team = pair / (wide * G4), members = a.H - team * G4 < G4 ? a.H - team * G4 : G4;
-        pair -= team * wide * G4;
-        const int place = pair / members;
-        h = team * G4 + pair - place * members;
-        rank = row * 8 + place;
-    }
+    const RaggedDeal deal = ragged_deal(a, total, part.n, blockIdx.x);
+    if (deal.rank < 0) return;
+    const int run = deal.run, h = deal.h, G = a.H / a.Hkv;
+    int rank = deal.rank;
     int r = -1, index = 0;
     if (few) {
-        // Longest walks first: blocks in descending order of their cost (stages, an estimate), ties by request.  Request i's blocks cost
-        // min(base + 2 b, cap), b = 0 .. blocks - 1 (a causal block of 256 rows sees two stages more than the one before), or cap each.
-        int base = 0, cap = 0;
-        if (blocks > 0) {
-            const int most = a.window > 0 ? (int)(((unsigned)a.window + (unsigned)a.sink + (a.causal ? 2 * KT : KT)) / KT) : 0x10000000;
-            cap = (mine.len + KT - 1) / KT;
-            base = a.causal ? cap - 2 * (blocks - 1) : cap;
-            cap = cap < most ? cap : most;
-        }
-        auto at_least = [&](int t) {  // blocks of this lane's request that cost t or more: the last ones
-            const int skip = a.causal ? (t - base + 1) >> 1 : t > base ? blocks : 0;
-            const int n = blocks - (skip > 0 ? skip : 0);
-            return t > cap || n < 0 ? 0 : n;
-        };
-        int lo = wave_least(blocks > 0 ? (base < cap ? base : cap) : 0x10000000), hi = wave_most(blocks > 0 ? cap : -0x10000000) + 1;
+        RaggedCost cost;  // longest walks first
+        cost.init<KT>(a, mine);
+        auto at_least = [&](int t) { return cost.at_least(t); };
+        int lo = wave_least(cost.least()), hi = wave_most(cost.most()) + 1;
         while (hi - lo > 1) {  // the cost of the block of this rank: the largest t with more than `rank` blocks of t or more
             const int mid = lo + ((hi - lo) >> 1);
             if (wave_total(at_least(mid)) > rank) lo = mid;
@@ -491,15 +446,8 @@ __global__ __launch_bounds__(256, 1) void attn_ragged_kernel(fvk_ragged_args a, 
     w.zstage = ks.n_sink - st0;
     w.zrows = ks.lo - ks.lo16;
     Groups<PAGED> grp;
+    grp.init(a, rq, st1, PAGED);
     grp.row = PAGED ? a.block_table + (long)r * a.table_width : nullptr;
-    grp.width = a.table_width;
-    grp.shift = PAGED ? a.page_shift : 0;
-    grp.n_pages = a.n_pages;
-    grp.end = st1;
-    grp.ps16 = (unsigned)(a.k_ps >> 3);
-    grp.rs16 = (unsigned)(a.k_rs >> 3);
-    grp.rs2 = rs2;
-    grp.base16 = (unsigned)rq.k0 * grp.rs16;
     grp.set(ks, st0, grp.load(ks, st0), w.grp_off, w.grp_rec);
 #define WAIT_ALL() asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #define BAR()                                   \
@@ -722,7 +670,7 @@ template <bool PAGED>
 int launch_blocks(const fvk_ragged_args* a, const RaggedParts& part, int n_blocks, hipStream_t s) {
     static FvkLdsConfigured configured;
     if (int rc = fvk_config_lds(configured, (const void*)attn_ragged_kernel<PAGED>, LDS_BYTES, "fvk_attn_ragged_bf16 (blocks)")) return rc;
-    hipLaunchKernelGGL((attn_ragged_kernel<PAGED>), dim3(8u * (a->H * (n_blocks / 8) * part.n + (a->H * (n_blocks % 8) * part.n + 7) / 8)), dim3(256), LDS_BYTES, s, *a, part);
+    hipLaunchKernelGGL((attn_ragged_kernel<PAGED>), dim3(ragged_grid(a->H, n_blocks, part.n)), dim3(256), LDS_BYTES, s, *a, part);
     FVK_LAUNCH_CHECK();
     return FVK_OK;
 }

@@ -106,30 +106,18 @@ __device__ __forceinline__ void attn_rows(const fvk_ragged_args& a, const Ragged
 
         auto issue = [&](int s, int slot) {
             const int k0 = ragged_stage<ST>(ks, s);
-            const int kmin = s < ks.n_sink ? 0 : ks.lo, kmax = s < ks.n_sink ? ks.sink_end : ks.hi;
+            const int kmin = s < ks.n_sink ? 0 : ks.lo, kmax = ragged_end(ks, s);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int key = k0 + 16 * half;
-                long kofs, vofs;
-                bool in_pool;
-                if (PAGED) {
-                    const int page = key < kmax ? pages.get(key >> a.page_shift) : -1, in_page = key & ((1 << a.page_shift) - 1);
-                    in_pool = page >= 0 && page < a.n_pages;
-                    kofs = in_pool ? (long)page * a.k_ps + (long)in_page * a.k_rs : 0;
-                    vofs = in_pool ? (long)page * a.v_ps + (long)in_page * a.v_rs : 0;
-                } else {
-                    in_pool = key < kmax;
-                    kofs = in_pool ? (long)key * a.k_rs : 0;
-                    vofs = in_pool ? (long)key * a.v_rs : 0;
-                }
-                const unsigned rec = in_pool ? 15 * (unsigned)(a.k_rs * 2) + 256 : 0, vrec = in_pool ? 15 * (unsigned)(a.v_rs * 2) + 256 : 0;
+                const RaggedHalf at16 = ragged_half<PAGED>(a, key, kmax, PAGED ? (key < kmax ? pages.get(key >> a.page_shift) : -1) : 0);
                 const unsigned dst = ragged_lds(ring) + slot * STAGE_BYTES + half * 4096;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int at = key + 4 * i + g;
                     const bool in = at >= kmin && at < kmax;
-                    ragged_dma((const unsigned char*)(kb + kofs), 0, rec, in ? k_off[i] : RAGGED_OUT, dst + i * 1024);
-                    ragged_dma((const unsigned char*)(vb + vofs), 0, vrec, in ? v_off[i & 1] + (unsigned)(4 * i * a.v_rs * 2) : RAGGED_OUT, dst + 8192 + i * 1024);
+                    ragged_dma((const unsigned char*)(kb + at16.k), 0, at16.k_rec, in ? k_off[i] : RAGGED_OUT, dst + i * 1024);
+                    ragged_dma((const unsigned char*)(vb + at16.v), 0, at16.v_rec, in ? v_off[i & 1] + (unsigned)(4 * i * a.v_rs * 2) : RAGGED_OUT, dst + 8192 + i * 1024);
                 }
             }
         };
@@ -155,7 +143,7 @@ __device__ __forceinline__ void attn_rows(const fvk_ragged_args& a, const Ragged
                     for (int qb = 0; qb < QB; ++qb) sc[qb][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[qb][c], sc[qb][t], 0, 0, 0);
                 }
             const int k0 = ragged_stage<ST>(ks, s);
-            const int kmin = s < ks.n_sink ? 0 : ks.lo, kmax = s < ks.n_sink ? ks.sink_end : ks.hi;
+            const int kmin = s < ks.n_sink ? 0 : ks.lo, kmax = ragged_end(ks, s);
             const bool full = k0 >= kmin && k0 + ST <= kmax && k0 + ST <= ks.full_hi && (s < ks.n_sink || k0 >= ks.full_lo);
             bf16x8 pf[QB];
             bool grew = false;
