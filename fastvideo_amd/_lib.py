@@ -20,7 +20,7 @@ PROBE = _PROBE_SEL == "1" or _PROBE_SEL.startswith("bug")
 # (scripts/coresidency/build_bug_strips.sh)
 LIB_PATH = (os.path.join(os.path.dirname(HERE), "scripts", "probes", f"libfvk_{_PROBE_SEL}.so" if _PROBE_SEL.startswith("bug") else "libfvk_probe.so")
             if PROBE else os.path.join(HERE, "libfvk_amd.so"))
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 vp, i32, i64, f32 = C.c_void_p, C.c_int, C.c_long, C.c_float
 
@@ -104,6 +104,7 @@ SIGNATURES = {
     "fvk_paged_plan": [vp] * 16 + [i32] * 10 + [vp],
     "fvk_rmsnorm_rope_paged_bf16": [vp] * 11 + [i32] * 3 + [i64] * 10 + [i32] * 9 + [f32, vp],
     "fvk_attn_ragged_workspace_bytes": [vp],
+    "fvk_attn_ragged_choice": [vp, C.POINTER(i32), C.POINTER(i32)],
     "fvk_attn_ragged_bf16": [vp, vp, i64, vp],
 }
 _RESTYPES = {"fvk_last_error": C.c_char_p, "fvk_attn_block_sparse_workspace_bytes": C.c_long, "fvk_attn_ragged_workspace_bytes": C.c_long}

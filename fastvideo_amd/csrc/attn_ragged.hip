@@ -24,6 +24,7 @@
 // Rounding: scores, sums and O in fp32; P to bf16 for the product with V (the matrix operand's type; the sum is taken of the rounded values, so the
 // weights add up to one); o once.
 #include "attn_ragged.h"
+#include "gemm_common.h"
 
 int fvk_attn_rows_launch(const fvk_ragged_args* a, int qb, long row_blocks, int n_split, float* o_part, float* lse_part, hipStream_t s);
 int fvk_ragged_merge_launch(const fvk_ragged_args* a, int n_split, float* o_part, float* lse_part, hipStream_t s);
@@ -705,6 +706,21 @@ Choice choose(const fvk_ragged_args* a) {
     const double part_us = (double)a->T * a->H * 1024 / 3.5e6;
     const bool may_split = (long)a->T * a->H <= 0xffffffL;  // the merge kernel's grid (2^32 threads)
     auto least = [](long x, long y) { return x < y ? x : y; };
+    // block kernel: 32-bit group offsets (16-byte units) and one descriptor stride for K and V are what its address registers hold
+    const long reach = a->block_table ? (a->n_pages > 0 ? a->n_pages - 1L : 0L) * a->k_ps + 256L * a->k_rs : (a->total_k + 1024L) * a->k_rs;
+    const long n_blocks = (a->T + 255L) / 256 + a->R - 1;  // the batch's blocks at most, whatever the lengths
+    const bool fits = a->k_ps == a->v_ps && a->k_rs == a->v_rs && a->k_ps >= 0 && reach / 8 <= 0xffffffffL && (n_blocks + 8) * a->H <= 0x7fffffL;
+    c.n_blocks = (int)n_blocks;
+#if FVK_VARIANTS  // the tests' choice: rows of a tile (16, 32, 64; 256: the block kernel) + 1024 * parts
+    if (const int forced = tunable(TUNE_ATTN_RAGGED)) {
+        const int tile = forced % 1024, most = tile == 256 ? 16 : 64;
+        c.blocks = tile == 256 && fits;
+        c.qb = tile < 64 ? tile / 16 : 4;
+        c.row_blocks = (rows + 16 * c.qb - 1) / (16 * c.qb);
+        c.n_split = may_split ? (int)least(forced / 1024, most) : 1;
+        return c;
+    }
+#endif
     double best = 0;
     for (int i = 0; i < 3; ++i) {
         const long tile = 16L << i, blocks = (rows + tile - 1) / tile;
@@ -728,12 +744,7 @@ Choice choose(const fvk_ragged_args* a) {
             c.n_split = (int)n;
         }
     }
-    // block kernel: 32-bit group offsets (16-byte units) and one descriptor stride for K and V are what its address registers hold
-    const long reach = a->block_table ? (a->n_pages > 0 ? a->n_pages - 1L : 0L) * a->k_ps + 256L * a->k_rs : (a->total_k + 1024L) * a->k_rs;
-    const bool fits = a->k_ps == a->v_ps && a->k_rs == a->v_rs && a->k_ps >= 0 && reach / 8 <= 0xffffffffL;
-    const long n_blocks = (a->T + 255L) / 256 + a->R - 1;  // the batch's blocks at most, whatever the lengths
-    c.n_blocks = (int)n_blocks;
-    if (!fits || (n_blocks + 8) * a->H > 0x7fffffL) return c;
+    if (!fits) return c;
     const long likely = least(least(a->R * ((max_q + 255) / 256), n_blocks), (a->T + 128L * a->R) / 256 + 1);
     const long stages = (max_kv + 127) / 128;
     for (long m = 1; m <= 16 && (m == 1 || (may_split && stages >= 3 * m && (n_blocks + 8) * a->H * m <= 0x7fffffL)); ++m) {
@@ -792,6 +803,16 @@ extern "C" long fvk_attn_ragged_workspace_bytes(const fvk_ragged_args* args) {
     if (a->T == 0) return 0;
     const Choice c = choose(a);
     return c.n_split > 1 ? (long)c.n_split * a->T * a->H * 129 * 4 : 0;
+}
+
+extern "C" int fvk_attn_ragged_choice(const fvk_ragged_args* args, int* tile, int* parts) {
+    FVK_CHECK(args && tile && parts, FVK_ERR_ARG, "fvk_attn_ragged_choice: null pointer");
+    const fvk_ragged_args b = plain(args), *a = &b;
+    if (int rc = check(a)) return rc;
+    const Choice c = choose(a);
+    *tile = c.blocks ? BMQ : 16 * c.qb;
+    *parts = c.n_split;
+    return FVK_OK;
 }
 
 extern "C" int fvk_attn_ragged_bf16(const fvk_ragged_args* args, void* ws, long ws_bytes, void* stream) {

@@ -15,7 +15,7 @@ void fvk_set_error(const char* fmt, ...) {
 }
 
 extern "C" const char* fvk_last_error(void) { return g_err; }
-extern "C" int fvk_abi_version(void) { return 9; }  // 9: + fvk_paged_plan, fvk_rmsnorm_rope_paged_bf16, fvk_attn_ragged_bf16, fvk_attn_ragged_workspace_bytes; 8: + fvk_attn_block_sparse_ws_bf16, fvk_attn_block_sparse_workspace_bytes (split last round of the 64-row list kernel); 7: + fvk_gemm_vt_bf16 (round 5's entry point, numbered in round 6), fvk_mfma_sustained_probe_bf16; 6: + fvk_qkv_norm_rope_pack2_bf16, dense kernel id 3 (attn_pp2 at any key length); 5: + fvk_attn_dense_kernel_bf16, fvk_attn_dense_split_bf16, fvk_qkvg_norm_rope_pack_bf16, fvk_is_probe_build
+extern "C" int fvk_abi_version(void) { return 10; }  // 10: + fvk_attn_ragged_choice; 9: + fvk_paged_plan, fvk_rmsnorm_rope_paged_bf16, fvk_attn_ragged_bf16, fvk_attn_ragged_workspace_bytes; 8: + fvk_attn_block_sparse_ws_bf16, fvk_attn_block_sparse_workspace_bytes (split last round of the 64-row list kernel); 7: + fvk_gemm_vt_bf16, fvk_mfma_sustained_probe_bf16; 6: + fvk_qkv_norm_rope_pack2_bf16, dense kernel id 3 (attn_pp2 at any key length); 5: + fvk_attn_dense_kernel_bf16, fvk_attn_dense_split_bf16, fvk_qkvg_norm_rope_pack_bf16, fvk_is_probe_build
 extern "C" int fvk_is_probe_build(void) { return FVK_VARIANTS; }
 
 extern "C" int fvk_device_arch(char* buf, int len) {
@@ -33,7 +33,7 @@ extern "C" int fvk_device_arch(char* buf, int len) {
 
 // ---- tunables (A/B switches for measurements; defaults = shipped configuration) ---------------------------------------
 static int g_tunables[fvk::TUNE_COUNT] = {0};
-static const char* const g_tunable_names[fvk::TUNE_COUNT] = {"gemm_impl", "attn_impl", "vae_conv_impl", "vsa_impl", nullptr};
+static const char* const g_tunable_names[fvk::TUNE_COUNT] = {"gemm_impl", "attn_impl", "vae_conv_impl", "vsa_impl", "attn_ragged", nullptr};
 
 #if FVK_VARIANTS
 int fvk::tunable(int id) { return (id >= 0 && id < fvk::TUNE_COUNT) ? g_tunables[id] : 0; }

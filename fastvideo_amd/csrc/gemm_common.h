@@ -56,7 +56,7 @@ int gemm_w1_fp8_launch(GemmArgs a, int epilogue, hipStream_t s);  // fvk_gemm_fp
 // the non-shipping kernels and schedules (attn_pp.hip, attn_vsa.hip, the attn_pp2 / gemm_ph / vae_conv3 variants, ablation probes) are
 // compiled in and `tunable()` reads the knob.  In the product library libfvk_amd.so FVK_VARIANTS is 0: every knob is the constant 0,
 // the variant dispatch is not compiled, and fvk_set_tunable accepts only the value 0.
-enum Tunable { TUNE_GEMM_IMPL = 0, TUNE_ATTN_IMPL = 1, TUNE_VAE_CONV_IMPL = 2, TUNE_VSA_IMPL = 3, TUNE_COUNT = 8 };
+enum Tunable { TUNE_GEMM_IMPL = 0, TUNE_ATTN_IMPL = 1, TUNE_VAE_CONV_IMPL = 2, TUNE_VSA_IMPL = 3, TUNE_ATTN_RAGGED = 4, TUNE_COUNT = 8 };
 #if FVK_VARIANTS  // fvk_common.h
 int tunable(int id);
 #else

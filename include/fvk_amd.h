@@ -27,7 +27,7 @@ extern "C" {
 #define FVK_ERR_LAUNCH (-2)  /* hipLaunch / hip runtime error                  */
 
 const char* fvk_last_error(void);
-int fvk_abi_version(void);                 /* bumps when a signature changes or entry points are added (5 = round 3, 6 = round 4, 7 = round 5's fvk_gemm_vt_bf16 + round 6's fvk_mfma_sustained_probe_bf16, 8 = fvk_attn_block_sparse_ws_bf16 / _workspace_bytes, fvk_block_mean_gather_bf16, 9 = fvk_paged_plan, fvk_rmsnorm_rope_paged_bf16, fvk_attn_ragged_bf16 / _workspace_bytes) */
+int fvk_abi_version(void);                 /* bumps when a signature changes or entry points are added (8 = fvk_attn_block_sparse_ws_bf16 / _workspace_bytes, fvk_block_mean_gather_bf16, 9 = fvk_paged_plan, fvk_rmsnorm_rope_paged_bf16, fvk_attn_ragged_bf16 / _workspace_bytes, 10 = fvk_attn_ragged_choice) */
 int fvk_device_arch(char* buf, int len);   /* gcnArchName of the current device ("gfx950...") */
 int fvk_is_probe_build(void);              /* 0: the product library; 1: the measurement build (scripts/probes/libfvk_probe.so) */
 /* Integer knobs for within-process A/B measurements (scripts/microbench.py); 0 = shipped configuration.
@@ -473,6 +473,8 @@ typedef struct {
     int causal, window, sink;
 } fvk_ragged_args;
 long fvk_attn_ragged_workspace_bytes(const fvk_ragged_args* a);
+/* Which kernel such a call takes: rows of a workgroup (16, 32, 64: the rows kernel; 256: the block kernel) and parts of the key axis. */
+int fvk_attn_ragged_choice(const fvk_ragged_args* a, int* tile, int* parts);
 int fvk_attn_ragged_bf16(const fvk_ragged_args* a, void* ws, long ws_bytes, void* stream);
 
 #ifdef __cplusplus
