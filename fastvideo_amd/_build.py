@@ -89,24 +89,62 @@ def build_probe(force: bool = False, verbose: bool = True) -> str:
 LAUNCH_LIB = os.path.join(HERE, "_launch.so")
 
 
+def launch_made_for() -> str:
+    """What a native front end belongs to: torch's C++ interface and CPython's have no stable ABI."""
+    import sys
+    import torch
+    return f"torch {torch.__version__}, Python {sys.version_info[0]}.{sys.version_info[1]}"
+
+
+def _launch_flags() -> list[str]:
+    import torch
+    return ["-O2", "-std=c++17", "-fPIC", "-shared", "-DNDEBUG", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            f'-DFVK_MADE_FOR="{launch_made_for()}"']
+
+
+def _launch_stamp() -> str:
+    """What the module was built for and with; no paths, so that it holds where the tree is copied to."""
+    return repr(_launch_flags())
+
+
+def launch_needs_build() -> bool:
+    """Missing, built for another torch or Python or with another command (its stamp beside it), or older than what it is built from."""
+    try:
+        with open(LAUNCH_LIB + ".flags") as f:
+            if f.read() != _launch_stamp():
+                return True
+    except OSError:
+        return True
+    deps = (os.path.join(CSRC, "launch.cpp"), os.path.join(HERE, "..", "include", "fvk_amd.h"))
+    return not os.path.exists(LAUNCH_LIB) or any(os.path.getmtime(LAUNCH_LIB) < os.path.getmtime(d) for d in deps)
+
+
 def build_launch(force: bool = False) -> str:
     """fastvideo_amd/_launch.so: the batched-cache operators' host side as a CPython module over torch's C++ tensors (csrc/launch.cpp; host code only)."""
-    src = os.path.join(CSRC, "launch.cpp")
-    deps = (src, os.path.join(HERE, "..", "include", "fvk_amd.h"))
-    if not force and os.path.exists(LAUNCH_LIB) and all(os.path.getmtime(LAUNCH_LIB) >= os.path.getmtime(d) for d in deps):
+    if not force and not launch_needs_build():
         return LAUNCH_LIB
+    import fcntl
     import sysconfig
     import torch
     root = os.path.dirname(torch.__file__)
-    part = f"{LAUNCH_LIB}.{os.getpid()}.o"   # (renamed when it is whole: several ranks may build at once)
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DNDEBUG", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
-           "-isystem", sysconfig.get_paths()["include"], src, "-o", part, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10"]
-    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"g++ failed on launch.cpp:\n{r.stdout}")
-    os.replace(part, LAUNCH_LIB)
-    return LAUNCH_LIB
+    with open(os.path.join(HERE, ".build.lock"), "w") as lock:   # one builder at a time, as above
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        try:
+            if not force and not launch_needs_build():
+                return LAUNCH_LIB
+            part = f"{LAUNCH_LIB}.{os.getpid()}.o"   # renamed when it is whole: a process that has the old one keeps it
+            cmd = ["g++", *_launch_flags(), "-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                   "-isystem", sysconfig.get_paths()["include"], os.path.join(CSRC, "launch.cpp"), "-o", part, "-L" + os.path.join(root, "lib"), "-ltorch_python",
+                   "-ltorch_cpu", "-ltorch", "-lc10"]
+            r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+            if r.returncode != 0:
+                raise RuntimeError(f"g++ failed on launch.cpp:\n{r.stdout}")
+            os.replace(part, LAUNCH_LIB)
+            with open(LAUNCH_LIB + ".flags", "w") as f:
+                f.write(_launch_stamp())
+            return LAUNCH_LIB
+        finally:
+            fcntl.flock(lock, fcntl.LOCK_UN)
 
 
 GUARD_LIB = os.path.join(PROBE_DIR, "libguard_alloc.so")

@@ -155,6 +155,10 @@ def launch():
             from . import _launch as module
         except ImportError as e:
             raise RuntimeError(f"fastvideo_amd/_launch.so does not load ({e}): run `python -c 'import __graft_entry__ as g; g.build()'`") from e
+        from . import _build
+        if module.made_for != _build.launch_made_for():
+            raise RuntimeError(f"fastvideo_amd/_launch.so was built for {module.made_for}, this is {_build.launch_made_for()}: run "
+                               "`python -c 'import __graft_entry__ as g; g.build()'`")
         module.init(*(C.cast(getattr(lib, name), vp).value for name in ("fvk_paged_plan", "fvk_rmsnorm_rope_paged_bf16", "fvk_attn_ragged_workspace_bytes",
                                                                         "fvk_attn_ragged_bf16", "fvk_last_error")))
         _native = module

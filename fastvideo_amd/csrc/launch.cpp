@@ -288,4 +288,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", nullptr, -1, methods, nu
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__launch() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__launch() {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "made_for", FVK_MADE_FOR) != 0) Py_CLEAR(m);  // neither torch's C++ interface nor CPython's has a stable ABI
+    return m;
+}
