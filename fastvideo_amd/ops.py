@@ -972,7 +972,8 @@ def rmsnorm_rope_paged(q, k, v, q_weight, k_weight, positions, rope, slot_map, k
     q [T, H*128], k / v [T, Hkv*128] bf16 row views (unit column stride); q_weight / k_weight bf16 or None (no norm); rope = (table fp32
     [n_t + n_h + n_w, pairs, 2], (n_t, n_h, n_w), (dim_t, dim_h, dim_w)) as rope.get_axis_rope builds it, or None (no rotation); positions int32 [T, 3]
     and slot_map int32 [T] from paged_plan.  Returns the rotated q [T, H*128] (``out``); k_pages / v_pages are written in place: rows whose slot is
-    negative or outside the pool are not.  A position outside the table gives a NaN row.  round_norm: the eager layer's two extra bf16 roundings."""
+    negative or outside the pool are not (a slot may occur once: of two rows that share one, keys and values may come from either).  A position outside
+    the table gives a NaN row.  round_norm: the eager layer's two extra bf16 roundings."""
     fast = _fast(k_pages)
     if fast is not None:
         got = _lib.launch().write(*fast, q, k, v, q_weight, k_weight, positions, rope, slot_map, k_pages, v_pages, eps, round_norm, out)

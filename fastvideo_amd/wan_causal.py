@@ -208,16 +208,20 @@ class CausalWanTransformer3DModelHip(WanTransformer3DModelHip):
         return ops.unpatchify(y.view(1, S, -1), (1, c_out, T, Hh, Wd), self.patch)
 
     # ------------------------------------------------------------------ several rollouts at once, over one pool of pages
+    def _paged_window(self, frame_seqlen: int):
+        if self.local_attn_size == -1:
+            return 0, 0
+        sink = self.sink_size * frame_seqlen
+        window = self.local_attn_size * frame_seqlen - sink
+        if window <= 0:
+            raise ValueError(f"sink_size={self.sink_size} leaves nothing of local_attn_size={self.local_attn_size}")
+        return window, sink
+
     def init_paged_cache(self, num_slots: int, num_pages: int, max_tokens: int, frame_seqlen: int, page_size: int = 64):
         """A pool for ``num_slots`` rollouts of this model.  The window is the one-sample path's: local_attn_size frames, the sink frames among them
         (the whole of a cache of local_attn_size frames, causal_wanvideo.py:123-173)."""
         from .paged_cache import PagedKVCache
-        window = sink = 0
-        if self.local_attn_size != -1:
-            sink = self.sink_size * frame_seqlen
-            window = self.local_attn_size * frame_seqlen - sink
-            if window <= 0:
-                raise ValueError(f"sink_size={self.sink_size} leaves nothing of local_attn_size={self.local_attn_size}")
+        window, sink = self._paged_window(frame_seqlen)
         return PagedKVCache(self.num_layers, self.H, num_slots, num_pages, max_tokens, page_size, window, sink, self.D, self.device)
 
     @torch.no_grad()
@@ -261,6 +265,8 @@ class CausalWanTransformer3DModelHip(WanTransformer3DModelHip):
         S, fs = math.prod(grid), grid[1] * grid[2]
         if self.local_attn_size == -1 and max(start_frames) + grid[0] > GLOBAL_ATTN_COMPAT_MAX_LATENT_FRAMES:
             raise ValueError(f"Causal Wan local_attn_size=-1 keeps {GLOBAL_ATTN_COMPAT_MAX_LATENT_FRAMES} latent frames; got a block to frame {max(start_frames) + grid[0]}")
+        if (cache.window_tokens, cache.sink_tokens) != self._paged_window(fs):
+            raise ValueError(f"forward_paged: a cache with a window of {cache.window_tokens} tokens behind {cache.sink_tokens} sinks is not one for frames of {fs} tokens")
         if text_kv[0][0].shape[0] != cache.num_slots * self.text_len:
             raise ValueError(f"forward_paged: text_kv holds {text_kv[0][0].shape[0]} states, {cache.num_slots} slots of {self.text_len} are needed")
         timestep = timestep.to(dev).reshape(R, -1)

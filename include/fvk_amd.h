@@ -444,7 +444,7 @@ int fvk_paged_plan(const int32_t* starts, const int32_t* new_lens, const int32_t
  * rope: fp32 [n_t + n_h + n_w, max(dim)/2, 2] = (cos, sin) per axis position and column pair, the axes one after another; dim_t + dim_h + dim_w = 128
  * columns of a head; NULL = no rotation.  positions int32 [T, 3]; a position outside the table gives a NaN row.
  * q_out [T, H*128]; k and v rows go to page slot_map[t] / page_size, row slot_map[t] % page_size (a negative slot or a page outside the pool: the row
- * is not written).  One rounding at the store; round_norm != 0: the normalised and the weighted value are rounded to bf16 as the eager layer does. */
+ * is not written; a slot may occur once: of two rows that share one, keys and values may come from either).  One rounding at the store; round_norm != 0: the normalised and the weighted value are rounded to bf16 as the eager layer does. */
 int fvk_rmsnorm_rope_paged_bf16(const void* q, const void* k, const void* v, const void* wq, const void* wk, const int32_t* positions,
                                 const float* rope, const int32_t* slot_map, void* q_out, void* k_pages, void* v_pages, int T, int H, int Hkv,
                                 long q_stride, long k_stride, long v_stride, long out_stride, long k_page_stride, long k_row_stride,

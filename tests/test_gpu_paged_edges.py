@@ -68,3 +68,22 @@ def test_blocks_whose_products_leave_fp32_with_both_signs(ops):
     assert torch.isfinite(o).all()
     assert ((o.double().cpu() - want).abs() <= tol + 128 * 2.0**-24 * 60 * 2 * vp.abs().max().item()).all()
     assert ((lse.double().cpu() - want_lse).abs() <= ref.LSE_TOL + 128 * 2.0**-24 * 60 * 2).all()
+
+
+# ------------------------------------------------------------------ the model's batched forward
+def test_a_cache_of_another_frame_size_is_refused(golden_dir):
+    """A cache's window and sinks are counted in tokens of one frame size; frames of another would be cut in their middle.  Nothing has changed then."""
+    import os
+    from fastvideo_amd.wan_causal import CausalWanTransformer3DModelHip
+    fx = torch.load(os.path.join(golden_dir, "wan_causal.pt"), weights_only=True)
+    case, fs = fx["cases"][1], fx["frame_seqlen"]
+    model = CausalWanTransformer3DModelHip(fx["state_dict"], num_heads=fx["config"]["num_heads"], local_attn_size=case["local_attn_size"],
+                                           sink_size=case["sink_size"], rope_cache_policy="absolute", num_frames_per_block=2)
+    c = case["calls"][0]
+    lat, t, text = c["latent"].cuda(), c["timestep"].cuda(), model.text_kv([case["ctx"]])
+    for size in (fs // 2, 2 * fs):
+        cache = model.init_paged_cache(1, 20, 8 * fs, size, 16)
+        with pytest.raises(ValueError, match=f"frames of {fs} tokens"):
+            model.forward_paged(lat, text, t, cache, [0])
+        assert cache.tokens == [0] and cache.free_page_count() == 20
+    assert torch.isfinite(model.forward_paged(lat, text, t, model.init_paged_cache(1, 20, 8 * fs, fs, 16), [0])).all()
