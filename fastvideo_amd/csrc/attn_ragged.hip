@@ -17,10 +17,10 @@
 //   * masks: sub-tiles that every row of the workgroup sees whole run a loop without a mask; the few at the edges of the window, at the sinks and on the
 //     diagonal run the same step with one.
 //   * the batch is packed: a workgroup finds its request from cu_q by a prefix sum over the lanes.
-// Measured (12 heads): 4680 rows over 32 760 keys 820 .. 840 us = 1.15 PFLOP/s (a large matrix product: 1.32), 0.60 of the cycles of the resident waves in the
+// Measured (12 heads; by card and clock): 4680 rows over 32 760 keys 793 .. 865 us = 1.09 .. 1.19 PFLOP/s (a large matrix product: 1.32), 0.60 of the cycles of the resident waves in the
 // matrix pipe, 228 of 256 compute units busy (19 blocks of 256 rows x 12); a pair of sub-tiles takes 7200 cycles, 4570 of them MFMA, and without the softmax
-// 5640, without the DMA 5970, without the LDS fragment reads 6470.  Four rollouts with a window of 9360 keys and 1560 sinks 400 us = 0.93 PFLOP/s, a causal prompt of ragged
-// requests 290 us = 0.84, 3 x 4680 rows over 512 text keys 71 us = 0.62 (set-up, first loads and store are half of a four-stage walk).
+// 5640, without the DMA 5970, without the LDS fragment reads 6470.  Four rollouts with a window of 9360 keys and 1560 sinks 390 .. 411 us = 0.90 .. 0.95 PFLOP/s, causal prompts of
+// ragged requests, 16 heads on 4, 287 .. 298 us = 0.82 .. 0.85, 3 x 4680 rows over 512 text keys 72 us = 0.61 (set-up, first loads and store are half of a four-stage walk).
 // Rounding: scores, sums and O in fp32; P to bf16 for the product with V (the matrix operand's type; the sum is taken of the rounded values, so the
 // weights add up to one); o once.
 #include "attn_ragged.h"
@@ -244,8 +244,8 @@ struct Wave {
     // One step of the pipeline.  Iteration t = 2j + 1 + EVEN of pair j: P V of sub-tile t-1 (V stage j, half EVEN), then K Q^T of sub-tile t+1 (K stage
     // j + 1, half EVEN); the vector stream is the softmax of sub-tile t.  LDS fragments are read FD ahead, each feeds four MFMAs; EVEN = 0 issues the
     // set {K(j+2), V(j+1)}, one piece every eighth MFMA.  The first step has no P V (and K in the other slot), the last one no K Q^T.
-    // Empty asm statements that READ a chunk's values keep its work in the chunk.  (As in-out operands they cost a padding s_nop in front of every reader: 74
-    // of a pair's 2600 instructions.)
+    // Empty asm statements that READ a chunk's values keep its work in the chunk.  (As in-out operands they cost a padding s_nop in front of every reader;
+    // the loop without masks has 1010 instructions a pair, 272 of them MFMAs.)
     template <int EVEN, bool MASK, bool PV = true, bool QK = true>
     __device__ __forceinline__ void iter(const Edges& e, int st0, int j) {
         constexpr int CUR = 1 - EVEN, FD = 6, PVS = PV ? 18 : 0, SLOTS = PVS + (QK ? 16 : 0), FRAGS = (PV ? 16 : 0) + (QK ? 16 : 0);
@@ -732,7 +732,7 @@ Choice choose(const fvk_ragged_args* a) {
             const long wgs = tiles * n, all = (long)a->R * a->Hkv, streams = least(all * n, i < 2 ? 512 : 256);
             // one stage per wave: two workgroups of the smaller tiles share a compute unit
             const double again = ((wgs + 255) / 256 - 1) * (i < 2 && max_kv <= 128 * n ? 0.5 : 1.0);
-            // several requests: unequal lengths even out over a few rounds (32 streams of 500 .. 16 000 keys: 206 us with 1024 workgroups, 278 with 256)
+            // several requests: unequal lengths even out over a few rounds (32 streams of 1500 .. 15 600 keys: 206 us with 1024 workgroups, 278 with 256)
             const double even = a->R == 1 || wgs <= 256 ? 1 : wgs >= 1024 ? 0.82 : 1 - 0.18 * (wgs - 256) / 768;
             const double part = ROWS_COST[i].key * max_kv / n * (1 + again * ROWS_COST[i].again);
             const double stream = all * max_kv * 512.0 * (1 + (tiles > all ? 0.054 * (tiles - all) / all : 0)) * (streams + 12.5) / (8.6e6 * streams);

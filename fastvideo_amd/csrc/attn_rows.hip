@@ -13,9 +13,10 @@
 // so neither the cache nor a pass over it holds a transposed copy.  P^T is the S^T registers of the same lane: lane (q = lane & 15, g = lane >> 4) holds keys
 // 4g..4g+3 of each 16-key tile, and the two tr reads of a V fragment fetch exactly those keys.
 // LDS images: K row r holds its 16-byte chunk c at c ^ (r & 15), V row r its 32-byte piece at piece ^ (r & 7): every fragment read touches all banks once.
-// Measured: one token over 900 keys, 12 heads, 6.2 us and 2.8 for the merge of its parts (launch latency); 32 streams over 500 .. 16 000 keys, 40 heads on 8,
-// 206 us (1.05 GB, 5.1 TB/s; a large copy reaches 4.8); 5 requests of 47 .. 186 rows over 1 .. 62 states, 12 heads, 10.2 us.
-// Rounding: scores, maximum, sum and O in fp32; P to bf16 for the product with V (the matrix operand's type; the sum is taken before that rounding); o once.
+// Measured: one token over 900 keys, 12 heads, 5.9 us and 2.9 for the merge of its parts (launch latency); 32 streams over 1500 .. 15 600 keys, 40 heads on 8,
+// 198 us and 4.7 (1.05 GB, 5.1 TB/s; a large copy reaches 4.8); 5 requests of 84 .. 186 rows over 0 .. 47 states, 12 heads, 10.1 us.
+// Rounding: scores, maximum, sum and O in fp32; P to bf16 for the product with V (the matrix operand's type; the sum is taken before that rounding, so a
+// row's weights add up to one within 2^-8; the block kernel's sum is taken after it); o once.
 #include "attn_ragged.h"
 
 namespace {

@@ -11,8 +11,8 @@ namespace {
 //   its i-th new page is free[count - 1 - off - i];  a page is dead once no row of this step or a later one can see it (window, sink) and goes back
 //   onto the stack in (request, page) order.
 // Bound: a few KB to a few MB, so launch latency; hence ONE launch for everything that does not depend on the number of dead pages (every workgroup
-// repeats the prefix sum over the requests: 2 loads and 8 shuffles for up to 256 of them, cheaper than a second launch), and a second one only when
-// there is a window.  Measured: 4.2 us for 16 streams of one token, 6.0 + 4.0 us for 48 rollouts of 150 000 tokens with a window (1000 cells a row).
+// repeats the prefix sums over the requests, tokens first, then the pages that the tokens within the batch need: cheaper than a second launch), and a second
+// one only when there is a window.  Measured: 4.2 us for 4 streams of one token, 6.2 + 4.2 us for 48 rollouts of 145 000 tokens with a window (1000 cells a row).
 struct PlanArgs {
     const int32_t *starts, *new_lens, *table, *held, *free_in, *count;
     int32_t *table_out, *held_out, *free_out, *count_out, *cu_q, *kv_lens, *slots, *positions, *granted;
@@ -275,7 +275,8 @@ __global__ __launch_bounds__(256) void paged_release_kernel(PlanArgs a) {
 // of a head are the same eight in every head (64 lanes x 8 columns = 4 heads per step), so its four (cos, sin) pairs are fetched once per row.
 // Rounded once, at the store; round_norm = 1 adds the two roundings of the eager layer (normalised value, weighted value), so that the batched path
 // caches the bits that the one-sample path caches.
-// Measured: 17.8 us for that block (4.9 TB/s; a large copy reaches 4.8), 153 us for 11 400 tokens of 40 heads (761 MB, 5.0 TB/s), 5.7 us for 16 tokens.
+// Measured: 17.7 us for that block (4.9 TB/s; a large copy reaches 4.8), 152 us for 12 390 tokens of 40 heads (761 MB, 5.0 TB/s), 5.6 us for 16 tokens; with
+// round_norm 0.4 .. 1.7 us more.
 struct WriteArgs {
     const bf16_t* in[3];
     const bf16_t* w[2];
@@ -416,7 +417,7 @@ extern "C" int fvk_paged_plan(const int32_t* starts, const int32_t* new_lens, co
     // (many requests: every workgroup repeats their prefix sum, so fewer of them; 4096 rows of 200 cells take 65 us, otherwise 141)
     const int row_waves = table_width > 64 && n_requests <= 1024 ? 4 : 1, table_blocks = (n_requests * row_waves + 3) / 4;
     const long items = n_tokens > n_free ? n_tokens : n_free;
-    // one item per thread up to half a million of them: a second one waits for its request and page again (150 000 tokens: 8.8 us with four, 6.1 with one)
+    // one item per thread up to half a million of them: a second one waits for its request and page again (145 000 tokens: 8.8 us with four, 6.1 with one)
     const long per = n_requests <= 1024 ? 256 : 1024;
     const int blocks = (int)((items + per - 1) / per < 2048 ? (items + per - 1) / per : 2048);
     PlanArgs a{starts, new_lens, block_table, pages_held, free_pages, free_count, table_out, held_out, free_out, count_out, cu_q, kv_lens, slot_map,

@@ -1,6 +1,7 @@
 """Causal (KV-cached) Wan2.1-1.3B rollout timing at 480p — not the contract bench.  21 latent frames in 7 blocks of 3, per block
 `--steps` DMD forwards + the clean-context re-run (CausalDMDDenosingStage's call pattern), KV cache of 21 frames (global attention).
-usage: python scripts/causal_bench.py [--steps 3] [--frames 21] [--local 0] [--sink 0]"""
+--rollouts R: R rollouts at once over one pool of pages (run_batch) against the same R one after the other.
+usage: python scripts/causal_bench.py [--steps 3] [--frames 21] [--local 0] [--sink 0] [--rollouts R]"""
 import argparse
 import json
 import os
@@ -15,6 +16,7 @@ ap.add_argument("--steps", type=int, default=3)
 ap.add_argument("--frames", type=int, default=21)
 ap.add_argument("--local", type=int, default=0, help="local_attn_size in frames (0 = global, 21-frame window)")
 ap.add_argument("--sink", type=int, default=0)
+ap.add_argument("--rollouts", type=int, default=0)
 args = ap.parse_args()
 
 import __graft_entry__ as G
@@ -26,7 +28,8 @@ dev = torch.device("cuda:0")
 cfg = WC.WAN21_T2V_1_3B
 sd = WC.random_state_dict(cfg, seed=0, device=dev)
 model = CausalWanTransformer3DModelHip(sd, cfg.num_heads, cfg.head_dim, cfg.patch_size, cfg.eps, cfg.freq_dim,
-                                       local_attn_size=(args.local or -1), sink_size=args.sink, num_frames_per_block=3, device=dev)
+                                       local_attn_size=(args.local or -1), sink_size=args.sink, num_frames_per_block=3, device=dev,
+                                       **(dict(rope_cache_policy="absolute") if args.rollouts else {}))
 del sd
 g = torch.Generator(device=dev).manual_seed(1)
 lat = torch.randn((1, 16, args.frames, 60, 104), generator=g, device=dev)
@@ -34,6 +37,26 @@ ctx = torch.randn((1, 512, cfg.text_dim), generator=g, device=dev).bfloat16()
 steps = [1000, 750, 500, 250][:args.steps]
 loop = CausalDenoisingLoopHip(model, steps)
 noise_fn = lambda shape, dtype: torch.randn(shape, generator=g, device=dev, dtype=torch.float32).to(dtype)
+if args.rollouts:
+    R, fwd = args.rollouts, args.frames // 3 * (len(steps) + 1)
+    lats, prompts = torch.randn((R, 16, args.frames, 60, 104), generator=g, device=dev), [ctx] * R
+
+    def timed(f):
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        out = f()
+        torch.cuda.synchronize()
+        assert torch.isfinite(out).all()
+        return (time.perf_counter() - t0) * 1e3
+
+    together = lambda: loop.run_batch(lats, prompts, noise_fn)
+    apart = lambda: torch.cat([loop.run(lats[r:r + 1], ctx, noise_fn) for r in range(R)])
+    loop.run_batch(lats[:, :, :6], prompts, noise_fn), loop.run(lat[:, :, :6], ctx, noise_fn)  # warm-up
+    ms = [(timed(together), timed(apart)) for _ in range(3)]   # in turn
+    best = [min(m[i] for m in ms) for i in range(2)]
+    print(json.dumps({"what": "causal Wan2.1-1.3B rollouts at once, 480p", "rollouts": R, "latent_frames": args.frames, "local": args.local, "sink": args.sink,
+                      "model_forwards_each": fwd, "together_ms": round(best[0], 1), "one_by_one_ms": round(best[1], 1), "ratio": round(best[1] / best[0], 3)}))
+    sys.exit(0)
 loop.run(lat[:, :, :6], ctx, noise_fn)  # warm-up (two blocks)
 torch.cuda.synchronize()
 model.attn_events = []
