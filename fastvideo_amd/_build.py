@@ -19,12 +19,12 @@ PROBE_LIB = os.path.join(PROBE_DIR, "libfvk_probe.so")
 # round 5, scripts/coresidency/coresidency_matrix.py only: the measurement build WITHOUT the two fences of round 4's co-residency bug (the register-file
 # claim of the one-wave-per-SIMD kernels, the packed-fp32 ban in the small kernels' files) — the pre-fix state, rebuilt on purpose to study it
 BUG_LIB = os.path.join(PROBE_DIR, "libfvk_bug.so")
-# The files of the SMALL kernels (norm / RoPE / pack, gathers, quantisers, scheduler step, post-processing: few registers, so their waves can
-# share a SIMD with another kernel's) are compiled WITHOUT packed-fp32 VALU instructions: round 4 found v_pk_mul_f32 / v_pk_add_f32 results of
-# such a wave wrong while a foreign MFMA stream ran on its SIMD (profiles/r04z_pk_f32_beside_mfma.log).  The known aggressors now
-# claim the whole register file; this is the second fence, for neighbours we do not control.  Same arithmetic (two scalar operations instead of
-# one packed one), and these kernels are HBM-bound.  (The host pass prints "not a recognized feature" for the flag: filtered below.)
-NO_PACKED_FP32 = ("norm_mod.hip", "vsa_misc.hip", "fp8.hip", "sched_step.hip", "vae_post.hip", "paged.hip", "attn_rows.hip", "attn_ragged.hip")
+# Every file is compiled WITHOUT packed-fp32 VALU instructions.  v_pk_mul_f32 / v_pk_add_f32 results of a wave have been wrong while a foreign MFMA stream ran
+# on its SIMD (profiles/r04z_pk_f32_beside_mfma.log), with no error, in ways that tests do not reliably show; hipcc makes them by itself from ordinary float
+# code.  Same arithmetic (two scalar operations instead of one packed one, the same roundings), and it costs nothing that can be measured: dense step 222.5 ms
+# with them in the GEMM, attention and convolution kernels, 222.7 without, VSA 147.9 / 148.1, sliding tile 127.8 / 127.7, VAE decode 234.9 / 235.6.
+# (The host pass prints "not a recognized feature" for the flag: filtered below.)
+NO_PACKED_FP32 = tuple(SOURCES + PROBE_SOURCES)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", "-Wno-unused-result"]
 FLAGS += os.environ.get("FVK_EXTRA_FLAGS", "").split()  # measurement builds only (e.g. -DFVK_ST_ABL=1 timing ablations)
 

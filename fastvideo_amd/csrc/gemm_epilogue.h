@@ -28,8 +28,7 @@ __device__ __forceinline__ float mul_then_add(float r, float y, float g) {
     return r + p;
 }
 
-// Two values at once: the multiplies / adds as packed fp32 operations (v_pk_mul_f32, v_pk_fma_f32, v_pk_add_f32 — the same IEEE results as the
-// scalar forms; a gain only where no MFMA runs beside them, i.e. in an exposed epilogue), the two transcendentals per value as before.
+// Two values at once: multiplies and adds in pairs (built as scalar operations: no packed fp32 in this library), the two transcendentals per value as before.
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x2_t gelu_tanh_fast2(f32x2_t x) {
     const float c0 = -2.0f * 0.7978845608028654f * 1.4426950408889634f;

@@ -107,7 +107,7 @@ __device__ __forceinline__ void w1_direct_epilogue(const fvk::GemmArgs& a, f32x4
                 }
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; e += 2) {  // (pairs: v_pk_add_f32 — the same sums)
+                for (int e = 0; e < 4; e += 2) {  // in pairs
                     const fvk::f32x2_t lo = fvk::f32x2_t{acc[2 * P][mb][e], acc[2 * P][mb][e + 1]} + fvk::f32x2_t{b8[e], b8[e + 1]};
                     const fvk::f32x2_t hi = fvk::f32x2_t{acc[2 * P + 1][mb][e], acc[2 * P + 1][mb][e + 1]} + fvk::f32x2_t{b8[4 + e], b8[5 + e]};
                     y[e] = (bf16_t)lo[0]; y[e + 1] = (bf16_t)lo[1];
