@@ -39,7 +39,7 @@ def test_the_rule_knows_such_a_load():
 
 
 def kernels(tmp_path, names):
-    """name -> (registers of a wave, spilled vector registers) of the built library's kernels."""
+    """name -> (registers of a wave, spilled vector registers, bytes of scratch) of the built library's kernels."""
     import subprocess
     import test_register_claims as claims
     objcopy, readelf = os.path.join(claims.LLVM, "llvm-objcopy"), os.path.join(claims.LLVM, "llvm-readelf")
@@ -53,13 +53,19 @@ def kernels(tmp_path, names):
         for blk in subprocess.run([readelf, "--notes", str(f)], capture_output=True, text=True).stdout.split("- .agpr_count:")[1:]:
             name = re.search(r"\.name:\s+(\S+)", blk).group(1)
             if any(n in name for n in names):
-                seen[name] = tuple(int(re.search(rf"\.{k}:\s+(\d+)", blk).group(1)) for k in ("vgpr_count", "vgpr_spill_count"))
+                seen[name] = tuple(int(re.search(rf"\.{k}:\s+(\d+)", blk).group(1)) for k in ("vgpr_count", "vgpr_spill_count", "private_segment_fixed_size"))
     return seen
 
 
 def test_rows_kernels_leave_no_room_beside_them(tmp_path):
     """One workgroup per compute unit (the two-stage ring, the 64-row tile): all 512 registers of a SIMD.  Two of them: half each."""
     ring = kernels(tmp_path, ["attn_rows_ring_kernel"])
-    assert len(ring) == 6 and all(v == (512, 0) for v in ring.values()), ring
+    assert len(ring) == 6 and all(v == (512, 0, 0) for v in ring.values()), ring
     one = kernels(tmp_path, ["attn_rows_kernel"])
-    assert len(one) == 6 and all(v == ((512 if "ILi4E" in n else 256), 0) for n, v in one.items()), one
+    assert len(one) == 6 and all(v == ((512 if "ILi4E" in n else 256), 0, 0) for n, v in one.items()), one
+
+
+def test_the_block_kernel_keeps_its_state_in_registers(tmp_path):
+    """All 512 of them, no spilled vector register and no scratch memory, paged and packed."""
+    blocks = kernels(tmp_path, ["attn_ragged_kernel"])
+    assert len(blocks) == 2 and all(v == (512, 0, 0) for v in blocks.values()), blocks
