@@ -11,8 +11,8 @@ namespace {
 //   its i-th new page is free[count - 1 - off - i];  a page is dead once no row of this step or a later one can see it (window, sink) and goes back
 //   onto the stack in (request, page) order.
 // Bound: a few KB to a few MB, so launch latency; hence ONE launch for everything that does not depend on the number of dead pages (every workgroup
-// repeats the prefix sums over the requests, tokens first, then the pages that the tokens within the batch need: cheaper than a second launch), and a second
-// one only when there is a window.  Measured: 4.2 us for 4 streams of one token, 6.2 + 4.2 us for 48 rollouts of 145 000 tokens with a window (1000 cells a row).
+// repeats the prefix sums over the requests: 2 loads and 8 shuffles for up to 256 of them, cheaper than a second launch), and a second one only when there
+// is a window.  Measured: 4.2 us for 4 streams of one token, 6.2 + 4.2 us for 48 rollouts of 145 000 tokens with a window (1000 cells a row).
 struct PlanArgs {
     const int32_t *starts, *new_lens, *table, *held, *free_in, *count;
     int32_t *table_out, *held_out, *free_out, *count_out, *cu_q, *kv_lens, *slots, *positions, *granted;
@@ -64,59 +64,58 @@ __device__ __forceinline__ int plan_page(const PlanArgs& a, const PlanReq& q, in
 }
 
 // Exclusive prefix sums over the requests by the whole workgroup (256 threads): new tokens, clamped to n_tokens, into cu[0..R], and the pages that the
-// tokens within the batch need into off[0..R].
+// tokens within the batch need into off[0..R].  Both in one pass, which is right where the batch holds all tokens; where it does not, the pages again with
+// the tokens that are left (a pass that waits for the tokens' sums first costs 10 % at 4096 requests).
 __device__ void plan_scan(const PlanArgs& a, int* cu, int* off) {
     __shared__ long wsum_t[4];
     __shared__ int wsum_p[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     long base_t = 0;
     int base_p = 0;
-    for (int r0 = 0; r0 < a.R; r0 += 256) {
-        const int r = r0 + tid;
-        long t = 0;
-        if (r < a.R) {
-            const int n = a.new_lens[r];
-            t = n > 0 ? n : 0;
-        }
-        const long t0 = t;
+    for (int pass = 0; pass < 2; ++pass) {
+        for (int r0 = 0; r0 < a.R; r0 += 256) {
+            const int r = r0 + tid;
+            long t = 0;
+            int p = 0;
+            if (r < a.R) {
+                if (pass == 0) {
+                    const int n = a.new_lens[r];
+                    t = n > 0 ? n : 0;
+                }
+                p = plan_req(a, r, pass == 0 ? (int)(t < a.n_tokens ? t : a.n_tokens) : cu[r + 1] - cu[r]).need;
+            }
+            const long t0 = t;
+            const int p0 = p;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const long tu = __shfl_up(t, o, 64);
-            if (lane >= o) t += tu;
+            for (int o = 1; o < 64; o <<= 1) {
+                const long tu = __shfl_up(t, o, 64);
+                const int pu = __shfl_up(p, o, 64);
+                if (lane >= o) { t += tu; p += pu; }
+            }
+            if (lane == 63) { wsum_t[wave] = t; wsum_p[wave] = p; }
+            __syncthreads();
+            long bt = base_t;
+            int bp = base_p;
+            for (int w = 0; w < 4; ++w) {
+                if (w < wave) { bt += wsum_t[w]; bp += wsum_p[w]; }
+                base_t += wsum_t[w];
+                base_p += wsum_p[w];
+            }
+            if (r < a.R) {
+                const long c = bt + t - t0;
+                if (pass == 0) cu[r] = (int)(c < a.n_tokens ? c : a.n_tokens);
+                off[r] = bp + p - p0;
+            }
+            __syncthreads();
         }
-        if (lane == 63) wsum_t[wave] = t;
-        __syncthreads();
-        long bt = base_t;
-        for (int w = 0; w < 4; ++w) {
-            if (w < wave) bt += wsum_t[w];
-            base_t += wsum_t[w];
-        }
-        const long from = bt + t - t0 < a.n_tokens ? bt + t - t0 : a.n_tokens, to = bt + t < a.n_tokens ? bt + t : a.n_tokens;
-        int p = r < a.R ? plan_req(a, r, (int)(to - from)).need : 0;
-        const int p0 = p;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int pu = __shfl_up(p, o, 64);
-            if (lane >= o) p += pu;
-        }
-        if (lane == 63) wsum_p[wave] = p;
-        __syncthreads();
-        int bp = base_p;
-        for (int w = 0; w < 4; ++w) {
-            if (w < wave) bp += wsum_p[w];
-            base_p += wsum_p[w];
-        }
-        if (r < a.R) {
-            cu[r] = (int)from;
-            off[r] = bp + p - p0;
+        if (tid == 0) {
+            if (pass == 0) cu[a.R] = (int)(base_t < a.n_tokens ? base_t : a.n_tokens);
+            off[a.R] = base_p;
         }
         __syncthreads();
+        if (base_t <= a.n_tokens) return;  // (the same in all threads)
+        base_p = 0;
     }
-    if (tid == 0) {
-        cu[a.R] = (int)(base_t < a.n_tokens ? base_t : a.n_tokens);
-        off[a.R] = base_p;
-    }
-    __syncthreads();
 }
 
 __device__ __forceinline__ bool plan_granted(const PlanReq& q, int off, int count) { return q.fits && (q.need == 0 || (long)off + q.need <= count); }
@@ -414,7 +413,7 @@ extern "C" int fvk_paged_plan(const int32_t* starts, const int32_t* new_lens, co
     FVK_CHECK(grid_h >= 1 && grid_w >= 1 && (long)grid_h * grid_w <= 0x7fffffffL, FVK_ERR_ARG, "fvk_paged_plan: grid %d x %d", grid_h, grid_w);
     FVK_CHECK(window >= 0 && sink >= 0 && (window > 0 || sink == 0), FVK_ERR_ARG, "fvk_paged_plan: window=%d sink=%d (a sink needs a window)", window, sink);
     FVK_CHECK(window == 0 || dead_counts, FVK_ERR_ARG, "fvk_paged_plan: a window needs dead_counts [2 * n_requests + 1]");
-    // (many requests: every workgroup repeats their prefix sum, so fewer of them; 4096 rows of 200 cells take 65 us, otherwise 141)
+    // (many requests: every workgroup repeats their prefix sum, so fewer of them; 4096 rows of 200 cells take 62 us with a window, otherwise 141)
     const int row_waves = table_width > 64 && n_requests <= 1024 ? 4 : 1, table_blocks = (n_requests * row_waves + 3) / 4;
     const long items = n_tokens > n_free ? n_tokens : n_free;
     // one item per thread up to half a million of them: a second one waits for its request and page again (145 000 tokens: 8.8 us with four, 6.1 with one)
